@@ -117,7 +117,7 @@ class saved_in_8_bits(torch.autograd.graph.saved_tensors_hooks):
             packs = operators.packs
             if packs is not _ALL and (not packs or tensor.untyped_storage().data_ptr() not in packs) or not _on_gpu(tensor) or \
                     tensor.dtype not in _FLOATS or tensor.numel() < min_numel or tensor.dim() == 0 or tensor.shape[-1] < 32:
-                return tensor
+                return tensor.detach()    # (an operator's result would hold the operator, and so itself)
             return BlockTensor.pack(tensor), tensor.dtype
 
         def unpack(saved):

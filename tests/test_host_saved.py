@@ -148,3 +148,33 @@ def test_contexts_nest_and_end():
             F.gelu(x * 2)
     F.gelu(x * 2)
     assert len(Rounded.taken) == 1
+
+
+def test_results_that_are_left_alone_are_freed_with_their_graph():
+    class Sentinel:
+        freed = 0
+
+        def __del__(self):
+            Sentinel.freed += 1
+
+    x = rand(96, 96)
+    for hooks in (contextlib.nullcontext(), saved_in_8_bits(), saved_in_8_bits(min_numel=1)):
+        before = Sentinel.freed
+        with hooks:
+            y = torch.exp(x * 1.0)    # (saves its result)
+        y.grad_fn.metadata['sentinel'] = Sentinel()
+        del y
+        assert Sentinel.freed == before + 1
+
+
+def test_gradients_of_gradients_pass_through_what_is_left_alone():
+    x, w = rand(8, 16, seed=21), torch.nn.Parameter(rand(16, 16, seed=22, grad=False))
+
+    def second():
+        first, = torch.autograd.grad((torch.exp(x @ w) * x).sum(), x, create_graph=True)
+        return torch.autograd.grad(first.square().sum(), (x, w))
+
+    want = second()
+    with saved_in_8_bits():
+        got = second()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
