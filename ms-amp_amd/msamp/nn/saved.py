@@ -117,11 +117,18 @@ class saved_in_8_bits(torch.autograd.graph.saved_tensors_hooks):
             packs = operators.packs
             if packs is not _ALL and (not packs or tensor.untyped_storage().data_ptr() not in packs) or not _on_gpu(tensor) or \
                     tensor.dtype not in _FLOATS or tensor.numel() < min_numel or tensor.dim() == 0 or tensor.shape[-1] < 32:
-                return tensor.detach()    # (an operator's result would hold the operator, and so itself)
+                # (detached: an operator's result would hold the operator, and so itself.  Autograd takes no note of versions behind hooks.)
+                return tensor.detach(), tensor._version
             return BlockTensor.pack(tensor), tensor.dtype
 
         def unpack(saved):
-            return saved if isinstance(saved, torch.Tensor) else saved[0].to(saved[1])
+            held, what = saved
+            if not isinstance(held, torch.Tensor):
+                return held.to(what)
+            if held._version != what:
+                raise RuntimeError('a tensor that the backward pass needs has been modified by an in-place operation: its shape is '
+                                   f'{tuple(held.shape)}, it is at version {held._version}, expected version {what}.')
+            return held
 
         super().__init__(pack, unpack)
 

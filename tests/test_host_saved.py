@@ -178,3 +178,28 @@ def test_gradients_of_gradients_pass_through_what_is_left_alone():
     with saved_in_8_bits():
         got = second()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_changes_in_place_are_noticed():
+    """Of what is left alone, as without the context; what was packed is what it was when it was saved."""
+    for hooks in (contextlib.nullcontext(), saved_in_8_bits(), saved_in_8_bits(min_numel=1)):
+        x, mask = rand(96, 96), torch.ones(96, 96)
+        with hooks:
+            y = x * 1.0 * mask
+        mask.add_(1.0)
+        with pytest.raises(RuntimeError, match='in-?place'):
+            y.sum().backward()
+        w = torch.nn.Parameter(rand(96, 96, grad=False))
+        with hooks:
+            y = F.linear(x * 1.0, w)
+        with torch.no_grad():
+            w.add_(1.0)    # (an optimizer's step between the forward and the backward pass)
+        with pytest.raises(RuntimeError, match='in-?place'):
+            y.sum().backward()
+    x = rand(96, 96)
+    with saved_in_8_bits(min_numel=1):
+        h = x * 2.0
+        y = F.gelu(h)
+    want, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    h.detach().zero_()
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
