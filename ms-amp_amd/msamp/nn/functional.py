@@ -217,31 +217,45 @@ class _FP8FusedLinearFunction(torch.autograd.Function):
         if bias is not None and not (bias.dtype == output_dtype and bias.is_contiguous()):
             bias = bias.detach().to(output_dtype).contiguous()
         src, meta = input.contiguous(), metas['input']
-        ctx.z = ctx.gate = None
+        z = g = None
         keeps = differentiable and (activation is not None or gate is not None)
         if _casts_in_one_call(src, meta, weight, output_dtype, bias):
             (n, m), device = (src.shape[0], weight.shape[0]), src.device
             gate = None if gate is None else Gemm._beside_output(gate, 'gate', n, m, output_dtype)
             residual = None if residual is None else Gemm._beside_output(residual, 'residual', n, m, output_dtype)
             if keeps:
-                ctx.z = BlockTensor._empty((n, m), device)
-                ctx.gate = None if gate is None else BlockTensor._empty((n, m), device)
-            out, ctx.input_codes, ctx.weight_codes, ctx.weight_words = _backend.linear_forward_fused(
+                z = BlockTensor._empty((n, m), device)
+                g = None if gate is None else BlockTensor._empty((n, m), device)
+            out, input_codes, weight_codes, words = _backend.linear_forward_fused(
                 src, meta, weight.value, weight.meta, output_dtype, bias, _backend.activation_code(activation), gate, residual,
-                (0, 0) if ctx.z is None else ctx.z._pointers(), (0, 0) if ctx.gate is None else ctx.gate._pointers()
+                (0, 0) if z is None else z._pointers(), (0, 0) if g is None else g._pointers()
             )
-            return out
-        input_fp8, weight_fp8 = src.cast(Dtypes.kfloat8_e4m3, meta=meta), weight.cast(Dtypes.kfloat8_e4m3)
-        ctx.input_codes, ctx.weight_codes, ctx.weight_words = input_fp8.value, weight_fp8.value, weight_fp8.meta
-        out = Gemm.fp8_gemm_fused(weight_fp8, input_fp8, Dtypes.dtype_to_qtype[output_dtype], bias=bias, activation=activation, gate=gate,
-                                  residual=residual, checkpoint=keeps)
-        if keeps:
-            out, ctx.z, ctx.gate = out
+            ctx.weight_meta = None
+        else:
+            input_fp8, weight_fp8 = src.cast(Dtypes.kfloat8_e4m3, meta=meta), weight.cast(Dtypes.kfloat8_e4m3)
+            input_codes, weight_codes, words, ctx.weight_meta = input_fp8.value, weight_fp8.value, None, weight_fp8.meta
+            out = Gemm.fp8_gemm_fused(weight_fp8, input_fp8, Dtypes.dtype_to_qtype[output_dtype], bias=bias, activation=activation, gate=gate,
+                                      residual=residual, checkpoint=keeps)
+            if keeps:
+                out, z, g = out
+        # (what autograd saves is freed behind the backward pass, attributes live as long as the output does)
+        ctx.save_for_backward(input_codes, weight_codes, words, None if z is None else z._buffer, None if g is None else g._buffer)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, output_grad):
+        ctx.input_codes, ctx.weight_codes, words, z, gate = ctx.saved_tensors
+        ctx.weight_words = ctx.weight_meta if words is None else words
+        shape, device = output_grad.shape, output_grad.device
+        ctx.z, ctx.gate = (None if buffer is None else BlockTensor._empty(shape, device, buffer=buffer) for buffer in (z, gate))
+        try:
+            return _FP8FusedLinearFunction._gradients(ctx, output_grad)
+        finally:
+            del ctx.input_codes, ctx.weight_codes, ctx.weight_words, ctx.z, ctx.gate
+
+    @staticmethod
+    def _gradients(ctx, output_grad):
         need_gate_grad, need_residual_grad = ctx.needs_input_grad[6], ctx.needs_input_grad[7]
         gate_grad = bias_grad = input_grad = None
         (tokens, d_out), d_in, meta = output_grad.shape, ctx.d_in, ctx.metas['ograd']

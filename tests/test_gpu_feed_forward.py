@@ -316,3 +316,35 @@ def test_saved_in_8_bits_around_fp8_layers():
     want, held = saved_gradients(lambda x: block(norm(x * 2.0), residual=x), (x, ), False)
     got, held8 = saved_gradients(lambda x: block(norm(x * 2.0), residual=x), (x, ), True)
     assert held8 < held and rel_fro(got[0], want[0]) < 3 * E4M3_RMS
+
+
+@pytest.mark.parametrize('d_in,d_out', [(1024, 4096), (1000, 4000)])
+def test_backward_frees_what_the_forward_pass_kept(d_in, d_out):
+    """While the output is still referenced, as a training loop's last loss is through the next forward pass."""
+    tokens = 2048
+    layer = fp8_layer(d_in, d_out, torch.bfloat16)
+    x = torch.randn(tokens, d_in, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    gate = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16)
+    kept = []
+    for _ in range(3):    # (the first time brings the gradients and workspaces)
+        before = torch.cuda.memory_allocated()
+        y = layer(x, activation='silu', gate=gate)
+        after = torch.cuda.memory_allocated()
+        y.backward(dy, retain_graph=True)
+        first = x.grad.clone()
+        x.grad = None
+        y.backward(dy)
+        assert torch.equal(x.grad, first)    # (the checkpoints are there for as long as the graph is)
+        first = None
+        kept.append((after - before, torch.cuda.memory_allocated() - before))
+        with pytest.raises(RuntimeError):
+            y.backward(dy)
+        x.grad = gate.grad = None
+        layer.weight.grad = layer.bias.grad = None
+        y_bytes, y = y.numel() * y.element_size(), None
+        torch.cuda.synchronize()
+    grads = x.numel() * 2 + gate.numel() * 2 + layer.weight.numel() + d_out * 4
+    codes = tokens * d_out * 2 * 33 // 32
+    held, left = kept[-1]
+    assert held > codes and left < y_bytes + grads + (1 << 20)
