@@ -621,12 +621,13 @@ enum {
  * (448 * 2^E), held to -126 .. 120; values are rounded to nearest, ties to even; NaN and the infinities become NaN; codes past
  * `cols` are zero.  Codes are 16-byte aligned. */
 #define MSAMP_CKPT_BLOCK 32
+#define MSAMP_CKPT_COLS 0x7fffffe0 /* columns at most */
 
 /* x: rows `row_stride` elements apart, F32 / F16 / BF16. */
-int msamp_checkpoint_pack(const void* x, int dtype, long long rows, int cols, long long row_stride, uint8_t* codes, uint8_t* exponents,
+int msamp_checkpoint_pack(const void* x, int dtype, long long rows, long long cols, long long row_stride, uint8_t* codes, uint8_t* exponents,
                           msamp_stream_t stream);
 /* out: [rows][cols], F32 / F16 / BF16, rounded once. */
-int msamp_checkpoint_unpack(const uint8_t* codes, const uint8_t* exponents, long long rows, int cols, void* out, int dtype,
+int msamp_checkpoint_unpack(const uint8_t* codes, const uint8_t* exponents, long long rows, long long cols, void* out, int dtype,
                             msamp_stream_t stream);
 
 /* d[n][m] = act(z) * gate + residual with z = (b[n][k] . a[m][k]^T) * a_scale_inv * b_scale_inv + bias, rounded once to d_dtype;
@@ -658,7 +659,7 @@ typedef struct msamp_gemm_fused_args {
 } msamp_gemm_fused_args;
 int msamp_fp8_gemm_fused(const msamp_gemm_fused_args* args, msamp_stream_t stream);
 int msamp_fp8_gemm_fused_pitch(long long m, long long n, long long k, long long* pitch);
-int msamp_pad_codes(const uint8_t* a, long long a_rows, uint8_t* a_out, const uint8_t* b, long long b_rows, uint8_t* b_out, int k,
+int msamp_pad_codes(const uint8_t* a, long long a_rows, uint8_t* a_out, const uint8_t* b, long long b_rows, uint8_t* b_out, long long k,
                     msamp_stream_t stream);
 
 /* msamp_linear_forward with msamp_fp8_gemm_fused in the place of the product: the casts of x and of the weight (whose codes are wanted
@@ -695,7 +696,7 @@ typedef struct msamp_activation_backward_args {
     int64_t scratch_bytes;
     void* workspace;
 } msamp_activation_backward_args;
-int msamp_activation_backward_scratch(int rows, int cols, int want_bias, int fp8, size_t* bytes);
+int msamp_activation_backward_scratch(long long rows, long long cols, int want_bias, int fp8, size_t* bytes);
 int msamp_activation_backward(const msamp_activation_backward_args* args, msamp_stream_t stream);
 
 #ifdef __cplusplus

@@ -537,38 +537,41 @@ using namespace msamp;
 
 extern "C" {
 
-int msamp_checkpoint_pack(const void* x, int dtype, long long rows, int cols, long long row_stride, uint8_t* codes, uint8_t* exponents,
+int msamp_checkpoint_pack(const void* x, int dtype, long long rows, long long cols, long long row_stride, uint8_t* codes, uint8_t* exponents,
                           msamp_stream_t stream) {
     MSAMP_REQUIRE(is_hp(dtype), MSAMP_ERR_DTYPE, "msamp_checkpoint_pack: dtype %d", dtype);
-    MSAMP_REQUIRE(rows >= 0 && cols >= 0 && (rows <= 1 || row_stride >= cols), MSAMP_ERR_SHAPE,
-                  "msamp_checkpoint_pack: %lld x %d, rows %lld apart", rows, cols, row_stride);
+    MSAMP_REQUIRE(rows >= 0 && cols >= 0 && cols <= MSAMP_CKPT_COLS && (rows <= 1 || row_stride >= cols), MSAMP_ERR_SHAPE,
+                  "msamp_checkpoint_pack: %lld x %lld, rows %lld apart", rows, cols, row_stride);
     if (rows == 0 || cols == 0) return MSAMP_OK;
     MSAMP_REQUIRE(x && codes && exponents, MSAMP_ERR_NULL, "msamp_checkpoint_pack: null pointer");
     MSAMP_REQUIRE(aligned(codes, 16), MSAMP_ERR_ALIGNMENT, "msamp_checkpoint_pack: codes must be 16-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSAMP_DT_F32) return launch_pack(static_cast<const float*>(x), rows, cols, row_stride, codes, exponents, st);
-    if (dtype == MSAMP_DT_F16) return launch_pack(static_cast<const f16_t*>(x), rows, cols, row_stride, codes, exponents, st);
-    return launch_pack(static_cast<const bf16_t*>(x), rows, cols, row_stride, codes, exponents, st);
+    const int width = static_cast<int>(cols);
+    if (dtype == MSAMP_DT_F32) return launch_pack(static_cast<const float*>(x), rows, width, row_stride, codes, exponents, st);
+    if (dtype == MSAMP_DT_F16) return launch_pack(static_cast<const f16_t*>(x), rows, width, row_stride, codes, exponents, st);
+    return launch_pack(static_cast<const bf16_t*>(x), rows, width, row_stride, codes, exponents, st);
 }
 
-int msamp_checkpoint_unpack(const uint8_t* codes, const uint8_t* exponents, long long rows, int cols, void* out, int dtype,
+int msamp_checkpoint_unpack(const uint8_t* codes, const uint8_t* exponents, long long rows, long long cols, void* out, int dtype,
                             msamp_stream_t stream) {
     MSAMP_REQUIRE(is_hp(dtype), MSAMP_ERR_DTYPE, "msamp_checkpoint_unpack: dtype %d", dtype);
-    MSAMP_REQUIRE(rows >= 0 && cols >= 0, MSAMP_ERR_SHAPE, "msamp_checkpoint_unpack: %lld x %d", rows, cols);
+    MSAMP_REQUIRE(rows >= 0 && cols >= 0 && cols <= MSAMP_CKPT_COLS, MSAMP_ERR_SHAPE, "msamp_checkpoint_unpack: %lld x %lld", rows, cols);
     if (rows == 0 || cols == 0) return MSAMP_OK;
     MSAMP_REQUIRE(codes && exponents && out, MSAMP_ERR_NULL, "msamp_checkpoint_unpack: null pointer");
     MSAMP_REQUIRE(aligned(codes, 16), MSAMP_ERR_ALIGNMENT, "msamp_checkpoint_unpack: codes must be 16-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSAMP_DT_F32) return launch_unpack(codes, exponents, rows, cols, static_cast<float*>(out), st);
-    if (dtype == MSAMP_DT_F16) return launch_unpack(codes, exponents, rows, cols, static_cast<f16_t*>(out), st);
-    return launch_unpack(codes, exponents, rows, cols, static_cast<bf16_t*>(out), st);
+    const int width = static_cast<int>(cols);
+    if (dtype == MSAMP_DT_F32) return launch_unpack(codes, exponents, rows, width, static_cast<float*>(out), st);
+    if (dtype == MSAMP_DT_F16) return launch_unpack(codes, exponents, rows, width, static_cast<f16_t*>(out), st);
+    return launch_unpack(codes, exponents, rows, width, static_cast<bf16_t*>(out), st);
 }
 
-int msamp_activation_backward_scratch(int rows, int cols, int want_bias, int fp8, size_t* bytes) {
-    MSAMP_REQUIRE(rows > 0 && cols > 0, MSAMP_ERR_SHAPE, "msamp_activation_backward_scratch: %d x %d", rows, cols);
+int msamp_activation_backward_scratch(long long rows, long long cols, int want_bias, int fp8, size_t* bytes) {
+    MSAMP_REQUIRE(rows > 0 && cols > 0 && rows <= 0x7fffffffLL && cols <= MSAMP_CKPT_COLS, MSAMP_ERR_SHAPE,
+                  "msamp_activation_backward_scratch: %lld x %lld", rows, cols);
     MSAMP_REQUIRE(bytes != nullptr, MSAMP_ERR_NULL, "msamp_activation_backward_scratch: null pointer");
-    MSAMP_REQUIRE(!fp8 || cols <= MSAMP_ACT_CAST_COLS, MSAMP_ERR_SHAPE, "msamp_activation_backward_scratch: a cast of %d columns", cols);
-    const SlabGrid sg = slab_grid(rows, cols, slab_workgroups(false));    // (the larger of the two)
+    MSAMP_REQUIRE(!fp8 || cols <= MSAMP_ACT_CAST_COLS, MSAMP_ERR_SHAPE, "msamp_activation_backward_scratch: a cast of %lld columns", cols);
+    const SlabGrid sg = slab_grid(static_cast<int>(rows), static_cast<int>(cols), slab_workgroups(false));    // (the larger of the two)
     *bytes = 4 * ((want_bias ? static_cast<size_t>(sg.slabs) * cols : 0) + (fp8 ? static_cast<size_t>(sg.slabs) * sg.strips : 0));
     return MSAMP_OK;
 }
@@ -583,7 +586,7 @@ int msamp_activation_backward(const msamp_activation_backward_args* args, msamp_
                   "msamp_activation_backward: bias_sum_dtype %d", static_cast<int>(a.bias_sum_dtype));
     MSAMP_REQUIRE(a.activation >= MSAMP_ACT_NONE && a.activation <= MSAMP_ACT_SILU, MSAMP_ERR_DTYPE,
                   "msamp_activation_backward: activation %d", static_cast<int>(a.activation));
-    MSAMP_REQUIRE(a.rows > 0 && a.cols > 0 && a.rows <= 0x7fffffffLL && a.cols <= 0x7fffffe0LL && (a.rows == 1 || a.dy_stride >= a.cols),
+    MSAMP_REQUIRE(a.rows > 0 && a.cols > 0 && a.rows <= 0x7fffffffLL && a.cols <= MSAMP_CKPT_COLS && (a.rows == 1 || a.dy_stride >= a.cols),
                   MSAMP_ERR_SHAPE, "msamp_activation_backward: %lld x %lld, rows of dy %lld apart", static_cast<long long>(a.rows),
                   static_cast<long long>(a.cols), static_cast<long long>(a.dy_stride));
     MSAMP_REQUIRE(a.dy && a.z_codes && a.z_exponents && a.dz && (!gated || (a.gate_exponents && a.dgate)), MSAMP_ERR_NULL,
@@ -596,7 +599,7 @@ int msamp_activation_backward(const msamp_activation_backward_args* args, msamp_
                   "msamp_activation_backward: codes must be 16-byte aligned");
     if (fp8 || a.bias_sum != nullptr) {
         size_t need = 0;
-        const int rc = msamp_activation_backward_scratch(static_cast<int>(a.rows), static_cast<int>(a.cols), a.bias_sum != nullptr, fp8, &need);
+        const int rc = msamp_activation_backward_scratch(a.rows, a.cols, a.bias_sum != nullptr, fp8, &need);
         if (rc != MSAMP_OK) return rc;
         MSAMP_REQUIRE(a.scratch != nullptr && static_cast<size_t>(a.scratch_bytes) >= need && aligned(a.scratch, 4), MSAMP_ERR_WORKSPACE,
                       "msamp_activation_backward: scratch of %zu bytes required", need);

@@ -265,18 +265,18 @@ extern "C" int msamp_fp8_gemm_fused_pitch(long long m, long long n, long long k,
     return MSAMP_OK;
 }
 
-extern "C" int msamp_pad_codes(const uint8_t* a, long long a_rows, uint8_t* a_out, const uint8_t* b, long long b_rows, uint8_t* b_out, int k,
+extern "C" int msamp_pad_codes(const uint8_t* a, long long a_rows, uint8_t* a_out, const uint8_t* b, long long b_rows, uint8_t* b_out, long long k,
                                msamp_stream_t stream) {
-    MSAMP_REQUIRE(a_rows >= 0 && b_rows >= 0 && k > 0 && k <= kMostK, MSAMP_ERR_SHAPE, "msamp_pad_codes: %lld and %lld rows of %d", a_rows, b_rows, k);
+    MSAMP_REQUIRE(a_rows >= 0 && b_rows >= 0 && k > 0 && k <= kMostK, MSAMP_ERR_SHAPE, "msamp_pad_codes: %lld and %lld rows of %lld", a_rows, b_rows, k);
     MSAMP_REQUIRE((a && a_out) || a_rows == 0, MSAMP_ERR_NULL, "msamp_pad_codes: null pointer");
     MSAMP_REQUIRE((b && b_out) || b_rows == 0, MSAMP_ERR_NULL, "msamp_pad_codes: null pointer");
     MSAMP_REQUIRE(aligned(a_out, 16) && aligned(b_out, 16), MSAMP_ERR_ALIGNMENT, "msamp_pad_codes: outputs must be 16-byte aligned");
-    const int chunks = (k + 15) / 16, per = std::min(chunks, kPadThreads);
+    const int chunks = static_cast<int>((k + 15) / 16), per = std::min(chunks, kPadThreads);
     const long long rows = a_rows + b_rows, rows_at_once = kPadThreads / per;
     if (rows == 0) return MSAMP_OK;
     const long long blocks = (rows + rows_at_once - 1) / rows_at_once;
     MSAMP_REQUIRE(blocks <= 0x7fffffffLL, MSAMP_ERR_SHAPE, "msamp_pad_codes: %lld rows", rows);
-    hipLaunchKernelGGL(pad_codes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPadThreads), 0, static_cast<hipStream_t>(stream), a, a_rows, a_out, b, rows, b_out, k);
+    hipLaunchKernelGGL(pad_codes_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kPadThreads), 0, static_cast<hipStream_t>(stream), a, a_rows, a_out, b, rows, b_out, static_cast<int>(k));
     MSAMP_CHECK_LAUNCH("pad_codes_kernel");
     return MSAMP_OK;
 }

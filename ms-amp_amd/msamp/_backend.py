@@ -66,12 +66,12 @@ _SIGNATURES = {
     'msamp_linear_forward_scratch': ([_i, _i, _i, _vp], _i),
     'msamp_linear_backward_scratch': ([_i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp], _i),
     'msamp_linear_backward': ([ctypes.c_char_p, _vp], _i),
-    'msamp_checkpoint_pack': ([_vp, _i, ctypes.c_longlong, _i, ctypes.c_longlong, _vp, _vp, _vp], _i),
-    'msamp_checkpoint_unpack': ([_vp, _vp, ctypes.c_longlong, _i, _vp, _i, _vp], _i),
+    'msamp_checkpoint_pack': ([_vp, _i, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _vp, _vp, _vp], _i),
+    'msamp_checkpoint_unpack': ([_vp, _vp, ctypes.c_longlong, ctypes.c_longlong, _vp, _i, _vp], _i),
     'msamp_fp8_gemm_fused': ([ctypes.c_char_p, _vp], _i),
     'msamp_fp8_gemm_fused_pitch': ([ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _vp], _i),
-    'msamp_pad_codes': ([_vp, ctypes.c_longlong, _vp, _vp, ctypes.c_longlong, _vp, _i, _vp], _i),
-    'msamp_activation_backward_scratch': ([_i, _i, _i, _i, _vp], _i),
+    'msamp_pad_codes': ([_vp, ctypes.c_longlong, _vp, _vp, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp], _i),
+    'msamp_activation_backward_scratch': ([ctypes.c_longlong, ctypes.c_longlong, _i, _i, _vp], _i),
     'msamp_activation_backward': ([ctypes.c_char_p, _vp], _i),
     'msamp_mfma_probe': ([_vp, _vp, _i, _i, _i, _vp, _vp], _i),
     'msamp_set_small_tile_limit': ([_i], None),
@@ -724,6 +724,7 @@ _GEMM_FUSED = struct.Struct('@20q')             # msamp_gemm_fused_args
 _ACTIVATION_BACKWARD = struct.Struct('@24q')    # msamp_activation_backward_args
 ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'gelu_tanh': 3, 'silu': 4}
 CKPT_BLOCK = 32
+CKPT_COLS = 0x7fffffe0    # MSAMP_CKPT_COLS
 FUSED_ROWS = 64    # MSAMP_FUSED_ROWS
 ACT_CAST_COLS = 524288    # MSAMP_ACT_CAST_COLS
 
@@ -742,6 +743,8 @@ def checkpoint_pitch(cols):
 
 def checkpoint_empty(rows, cols, device):
     """Memory for a checkpoint: rows * pitch codes and behind them rows * pitch / 32 exponents."""
+    if cols > CKPT_COLS:
+        raise ValueError(f'a checkpoint has at most {CKPT_COLS} columns, not {cols}.')
     pitch = checkpoint_pitch(cols)
     return torch.empty((rows * (pitch + pitch // CKPT_BLOCK), ), dtype=torch.uint8, device=device)
 

@@ -19,6 +19,8 @@ class BlockTensor:
         blocks = (cols + _backend.CKPT_BLOCK - 1) // _backend.CKPT_BLOCK
         if value.dtype != torch.uint8 or exponent.dtype != torch.uint8:
             raise TypeError(f'codes and exponents should be torch.uint8, not {value.dtype} and {exponent.dtype}.')
+        if cols > _backend.CKPT_COLS:
+            raise ValueError(f'a checkpoint has at most {_backend.CKPT_COLS} columns, not {cols}.')
         if tuple(value.shape) != (rows, blocks * _backend.CKPT_BLOCK) or tuple(exponent.shape) != (rows, blocks):
             raise ValueError(f'codes {tuple(value.shape)} and exponents {tuple(exponent.shape)} do not hold a tensor of shape {tuple(shape)}.')
         if not (value.is_contiguous() and exponent.is_contiguous()):

@@ -6,6 +6,7 @@ import torch
 import torch.nn.functional as F
 from torch.overrides import TorchFunctionMode
 
+from msamp import _backend
 from msamp.common.tensor import BlockTensor
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -116,7 +117,7 @@ class saved_in_8_bits(torch.autograd.graph.saved_tensors_hooks):
         def pack(tensor):
             packs = operators.packs
             if packs is not _ALL and (not packs or tensor.untyped_storage().data_ptr() not in packs) or not _on_gpu(tensor) or \
-                    tensor.dtype not in _FLOATS or tensor.numel() < min_numel or tensor.dim() == 0 or tensor.shape[-1] < 32:
+                    tensor.dtype not in _FLOATS or tensor.numel() < min_numel or tensor.dim() == 0 or not 32 <= tensor.shape[-1] <= _backend.CKPT_COLS:
                 # (detached: an operator's result would hold the operator, and so itself.  Autograd takes no note of versions behind hooks.)
                 return tensor.detach(), tensor._version
             return BlockTensor.pack(tensor), tensor.dtype

@@ -1,6 +1,7 @@
 """Host side of the operators between two linear layers, without a GPU: argument blocks, constants, checks of arguments, and the
 oracle against what torch computes."""
 
+import ctypes
 import os
 import re
 
@@ -96,3 +97,24 @@ def test_saved_in_8_bits_leaves_tensors_outside_the_gpu_alone():
         y = (x * 2).exp().sum()
     y.backward()
     assert torch.allclose(x.grad, 2 * (2 * x).exp().detach())
+
+
+ERR_SHAPE = int(re.search(r'MSAMP_ERR_SHAPE = (-?\d+)', HEADER).group(1))
+
+
+def test_sizes_beyond_the_kernels_are_refused_and_not_cut():
+    """Sizes past 31 and 32 bits (the library refuses them before it looks at a pointer), in every call that takes one by value."""
+    assert int(re.search(r'#define MSAMP_CKPT_COLS (\w+)', HEADER).group(1), 16) == _backend.CKPT_COLS
+    lib, p, size = _backend.load(), 64, ctypes.c_size_t()
+    for cols in (_backend.CKPT_COLS + 1, 2**31, 2**32 + 64, 2**40):
+        assert lib.msamp_checkpoint_pack(p, _backend.DT_BF16, 1, cols, cols, p, p, None) == ERR_SHAPE
+        assert lib.msamp_checkpoint_unpack(p, p, 1, cols, p, _backend.DT_BF16, None) == ERR_SHAPE
+        assert lib.msamp_activation_backward_scratch(4, cols, 1, 0, ctypes.addressof(size)) == ERR_SHAPE
+        assert lib.msamp_activation_backward_scratch(cols + 2**31, 64, 1, 0, ctypes.addressof(size)) == ERR_SHAPE
+        assert lib.msamp_pad_codes(p, 1, p, p, 1, p, cols, None) == ERR_SHAPE
+        with pytest.raises(ValueError):
+            _backend.checkpoint_empty(1, cols, 'cpu')
+        with pytest.raises(ValueError):
+            BlockTensor(torch.zeros(1, 32, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8), (1, cols))
+        with pytest.raises(ValueError):
+            BlockTensor._empty((cols, ), 'cpu')
