@@ -473,9 +473,20 @@ __device__ __forceinline__ void k_part(In& X, In& Y, Out& D, int NR, int NC, int
     K = end - first;
 }
 
+// An output: nothing else points to it, but with the fused epilogue, where it may be the residual.
+template <typename OT, bool FUSED>
+struct OutputPointer {
+    using type = OT* __restrict__;
+};
+template <typename OT>
+struct OutputPointer<OT, true> {
+    using type = OT*;
+};
+
 //  * TAIL = Epilogue: the output is act(D) * gate + residual, rounded once, with checkpoints of D and of the gate beside it on demand.
 template <int XF, int YF, typename OT, bool XT, bool YT, int QF, bool QSPEC, bool KTAIL, typename TAIL>
-__device__ __forceinline__ void gemm_dma256(const uint8_t* __restrict__ X, const uint8_t* __restrict__ Y, OT* __restrict__ D, int NR, int NC, int K,
+__device__ __forceinline__ void gemm_dma256(const uint8_t* __restrict__ X, const uint8_t* __restrict__ Y,
+                                            typename OutputPointer<OT, std::is_same<TAIL, Epilogue>::value>::type D, int NR, int NC, int K,
                                             const float* __restrict__ x_scale_inv, const float* __restrict__ y_scale_inv, int accumulate,
                                             const void* __restrict__ bias, int bias_dt, const TAIL& qa) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];

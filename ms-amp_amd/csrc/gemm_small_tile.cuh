@@ -88,8 +88,8 @@ __device__ __forceinline__ v4f vacc_quad(uint32_t token) {
 }
 
 template <int XF, int YF, typename OT, bool XT, bool YT, bool KTAIL, bool PAIR = false, bool FUSED = false>
-__device__ __forceinline__ void gemm_dma128(const uint8_t* __restrict__ X, const uint8_t* __restrict__ Y, OT* __restrict__ D, int NR,
-                                            int NC, int K, const float* __restrict__ x_scale_inv,
+__device__ __forceinline__ void gemm_dma128(const uint8_t* __restrict__ X, const uint8_t* __restrict__ Y,
+                                            typename OutputPointer<OT, FUSED>::type D, int NR, int NC, int K, const float* __restrict__ x_scale_inv,
                                             const float* __restrict__ y_scale_inv, int accumulate, const void* __restrict__ bias,
                                             int bias_dt, const Epilogue* fused = nullptr) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+from msamp import _backend
 from msamp.common.dtype import Dtypes
 from msamp.common.tensor import BlockTensor, ScalingMeta, ScalingTensor
 from msamp.operators.activation import Activation
@@ -505,3 +506,27 @@ def test_operands_past_4_gib():
     dz, _, _ = Activation.backward_cast(many, z8, 'silu', meta, gate=g8, bias_dtype=torch.float32)
     assert abs(float(meta.amax[0]) - float(want_dz.abs().max())) <= 1e-5 * float(want_dz.abs().max())
     assert same_blocks(dz.value, block)
+
+
+# (few rows in 16-byte accesses and not; paired, small and large tiles; tiles of two sizes; rows that begin anywhere in tiles)
+@pytest.mark.parametrize('n,m,k', [(5, 96, 256), (48, 65, 1040), (130, 512, 512), (2048, 1024, 1024), (1024, 1032, 2064), (2304, 8192, 256), (4289, 4096, 4096),
+                                   (300, 72, 1040), (2500, 4101, 384), (150, 513, 1040)])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_fused_product_in_place_of_its_residual(n, m, k, dtype):
+    """The output may be the residual, in every kernel: the same bits as beside it."""
+    x, xs = whole_codes(n, k, 121)
+    w, ws = whole_codes(m, k, 122)
+    gate, residual = torch.randn(n, m, device='cuda').to(dtype), torch.randn(n, m, device='cuda').to(dtype)
+    bias, code = torch.randn(m, device='cuda').to(dtype), _backend.activation_code('gelu')
+    for g, checkpoint in ((None, False), (gate, True)):
+        outs = []
+        for in_place in (False, True):
+            old = residual.clone()
+            z8 = BlockTensor._empty((n, m), old.device) if checkpoint else None
+            g8 = BlockTensor._empty((n, m), old.device) if checkpoint else None
+            out = _backend.fp8_gemm_fused(ws.value, ws.meta.scale_inv, xs.value, xs.meta.scale_inv, old if in_place else torch.empty_like(old), bias, code, g, old,
+                                          (0, 0) if z8 is None else z8._pointers(), (0, 0) if g8 is None else g8._pointers())
+            assert (out.data_ptr() == old.data_ptr()) == in_place
+            outs.append([out] + ([z8.value, z8.exponent, g8.value, g8.exponent] if checkpoint else []))
+        for a, b in zip(*outs):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), (n, m, k, dtype, checkpoint)

@@ -111,3 +111,27 @@ def test_accumulators_are_read_behind_the_products(assembly, name):
 
 def test_every_kernel_is_looked_at(assembly):
     assert len(set(itertools.chain.from_iterable(assembly.values()))) == 18
+
+
+def test_output_may_be_the_residual(tmp_path):
+    """The fused forms promise the compiler nothing about what else points to their output; the others, whose outputs are their own, do."""
+    hipcc = shutil.which('hipcc') or '/opt/rocm/bin/hipcc'
+    if not os.path.exists(hipcc):
+        pytest.skip('no hipcc here')
+    src = os.path.join(os.path.dirname(_backend.__file__), '..', 'csrc')
+    common = [hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-Wno-unused-command-line-argument', '-Wno-inline-asm', '--cuda-device-only', '-S', '-emit-llvm',
+              '-Xclang', '-disable-llvm-passes']
+    seen = set()
+    for unit, defines in (('gemm_fused_tiles', ['-DMSAMP_FUSED_OT=bf16_t']), ('gemm_inst', ['-DMSAMP_XF=5', '-DMSAMP_YF=5'])):
+        out = str(tmp_path / f'{unit}.ll')
+        done = subprocess.run([*common, *defines, '-o', out, os.path.join(src, unit + '.hip')], cwd=src, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+        assert done.returncode == 0, done.stdout.decode(errors='replace')[-2000:]
+        for line in open(out):
+            m = re.match(r'define .*@(_ZN5msamp11gemm_dma(?:256|128)I\w+)\(([^)]*)\)', line)
+            if not m:
+                continue
+            x, y, d = m.group(2).split(', ')[:3]
+            fused = unit == 'gemm_fused_tiles'
+            assert 'noalias' in x and 'noalias' in y and ('noalias' in d) != fused, (m.group(1), d)
+            seen.add((unit, 'dma256' in m.group(1)))
+    assert ('gemm_fused_tiles', True) in seen and ('gemm_fused_tiles', False) in seen and ('gemm_inst', True) in seen
