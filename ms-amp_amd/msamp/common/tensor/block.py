@@ -25,6 +25,8 @@ class BlockTensor:
             raise ValueError(f'codes {tuple(value.shape)} and exponents {tuple(exponent.shape)} do not hold a tensor of shape {tuple(shape)}.')
         if not (value.is_contiguous() and exponent.is_contiguous()):
             raise ValueError('The codes or the exponents are not contiguous.')
+        if value.device != exponent.device:
+            raise ValueError(f'The codes are on {value.device}, the exponents on {exponent.device}.')
         self._value, self._exponent, self._buffer = value, exponent, None
         self.shape, self._rows, self._cols = shape, rows, cols
 

@@ -20,6 +20,8 @@ class Activation:
             raise TypeError('z and the gate should be BlockTensors.')
         if not (output_grad.is_cuda and z.is_cuda and (gate is None or gate.is_cuda)):
             raise ValueError('The output gradient or a checkpoint is not in cuda memory.')
+        if z.device != output_grad.device or gate is not None and gate.device != output_grad.device:
+            raise ValueError('The output gradient and the checkpoints are on different devices.')
         if output_grad.dtype not in _FLOATS or bias_dtype not in _FLOATS + (None, ):
             raise TypeError(f'unsupported types: output gradient {output_grad.dtype}, bias gradient {bias_dtype}.')
         if output_grad.shape != z.shape or gate is not None and gate.shape != z.shape:
@@ -58,7 +60,8 @@ class Activation:
     @staticmethod
     def takes_cast(meta, cols):
         """True if backward_cast takes an output gradient of `cols` columns with this meta."""
-        return Dtypes.is_fp8_qtype(meta.qtype) and meta.scaling_mode() == 'gated' and meta.scale.is_cuda and 0 < cols <= _backend.ACT_CAST_COLS
+        return Dtypes.is_fp8_qtype(meta.qtype) and meta.scaling_mode() == 'gated' and 0 < cols <= _backend.ACT_CAST_COLS and \
+            meta.scale.is_cuda and meta.scale_inv.is_cuda and meta.amax.is_cuda
 
     @classmethod
     def backward_cast(cls, output_grad, z, activation, meta, gate=None, bias_dtype=None):

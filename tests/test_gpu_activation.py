@@ -530,3 +530,31 @@ def test_fused_product_in_place_of_its_residual(n, m, k, dtype):
             outs.append([out] + ([z8.value, z8.exponent, g8.value, g8.exponent] if checkpoint else []))
         for a, b in zip(*outs):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), (n, m, k, dtype, checkpoint)
+
+
+def test_operands_on_the_host_are_refused():
+    """All of them, before anything is launched: scales, exponents and parts of a meta as well as tensors."""
+    x, xs = whole_codes(4, 64, 131)
+    w, ws = whole_codes(8, 64, 132)
+    host = ScalingTensor(xs.value, ScalingMeta(Dtypes.kfloat8_e4m3, device='cpu'))
+    host_codes = ScalingTensor(xs.value.cpu(), xs.meta)
+    for a, b in ((ws, host), (host, ws), (ws, host_codes), (host_codes, ws)):
+        with pytest.raises(ValueError):
+            Gemm.fp8_gemm_fused(a, b, Dtypes.kbfloat16)
+    out = Gemm.fp8_gemm_fused(ws, xs, Dtypes.kbfloat16)
+    for beside in (dict(bias=out[0].cpu()), dict(gate=out.cpu()), dict(residual=out.cpu())):
+        with pytest.raises(ValueError):
+            Gemm.fp8_gemm_fused(ws, xs, Dtypes.kbfloat16, **beside)
+    z8, z = held(4, 64, 133)
+    dy = torch.randn(4, 64, device='cuda')
+    with pytest.raises(ValueError):
+        BlockTensor(z8.value, z8.exponent.cpu(), (4, 64))
+    on_host = BlockTensor(z8.value.cpu(), z8.exponent.cpu(), (4, 64))
+    for of, gate in ((on_host, None), (z8, on_host)):
+        with pytest.raises(ValueError):
+            Activation.backward(dy, of, 'gelu', gate=gate)
+    for name in ('scale', 'scale_inv', 'amax', 'amax_counter'):
+        meta = ScalingMeta(Dtypes.kfloat8_e5m2, window_size=16)
+        setattr(meta, name, getattr(meta, name).cpu())
+        with pytest.raises(ValueError):
+            Activation.backward_cast(dy, z8, 'gelu', meta)

@@ -118,3 +118,11 @@ def test_sizes_beyond_the_kernels_are_refused_and_not_cut():
             BlockTensor(torch.zeros(1, 32, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8), (1, cols))
         with pytest.raises(ValueError):
             BlockTensor._empty((cols, ), 'cpu')
+
+
+def test_codes_and_exponents_lie_on_one_device():
+    """(The codes alone used to be asked where they are, and kernels were given the address of exponents on the host.)"""
+    with pytest.raises(ValueError):
+        BlockTensor(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8, device='meta'), (4, 33))
+    with pytest.raises(ValueError):
+        BlockTensor(torch.zeros(4, 64, dtype=torch.uint8, device='meta'), torch.zeros(4, 2, dtype=torch.uint8), (4, 33))
