@@ -53,7 +53,7 @@ __device__ __forceinline__ void act_part(float z, float& part, float& slope) {
         part = normal_cdf(z);
         slope = fmaf(z * bell, 0.39894228040143268f, part);
     } else if constexpr (ACT == MSAMP_ACT_GELU_TANH) {
-        const float zz = z * z;
+        const float zz = fminf(z * z, 1e30f);    // (finite: behind it stands a factor of 0)
         part = tanh_part(z);
         slope = fmaf(z * part * (1.0f - part), fmaf(3.0f * kTanhTwice * kTanhCube, zz, kTanhTwice), part);
     } else {

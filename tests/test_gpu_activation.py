@@ -558,3 +558,26 @@ def test_operands_on_the_host_are_refused():
         setattr(meta, name, getattr(meta, name).cpu())
         with pytest.raises(ValueError):
             Activation.backward_cast(dy, z8, 'gelu', meta)
+
+
+@pytest.mark.parametrize('name', oact.NAMES)
+@pytest.mark.parametrize('gated', [False, True])
+def test_gradients_of_values_whose_square_leaves_float32(name, gated):
+    """Exponents up to the largest: a slope there is 0 or 1 (the oracle's, in 64 bits, as well), with a bias gradient and without."""
+    exponents = [139, 180, 187, 190, 191, 192, 200, 230, 239]
+    rows, cols = len(exponents), 256
+    codes = (torch.arange(256) & 0xfe).to(torch.uint8)    # (without the two NaN codes)
+    value, exponent = codes.repeat(rows, 1).cuda(), torch.tensor(exponents, dtype=torch.uint8)[:, None].expand(rows, cols // 32).contiguous().cuda()
+    z8 = BlockTensor(value, exponent, (rows, cols))
+    z = oact.unpack(value.cpu(), exponent.cpu(), cols)
+    assert bool(torch.isfinite(z).all()) and float(z.abs().max()) < 2.0**121 * 448
+    g8, g = held(rows, cols, 141) if gated else (None, None)
+    dy = torch.randn(rows, cols, generator=gen(142))
+    want_dz, want_dg, _ = oact.gradients(dy, z, name, g)
+    error = dy.double().abs() * (1.0 if g is None else g.abs()) * torch.where(z.abs() > 16.0, 1e-6, slope_error(z.clamp(-16.0, 16.0)))
+    for bias_dtype in (None, torch.float32):
+        dz, dg, db = Activation.backward(dy.cuda(), z8, name, gate=g8, bias_dtype=bias_dtype)
+        assert_within(dz, want_dz, allowed(torch.float32, want_dz, error + 2.0**-22 * want_dz.abs()), (name, gated, bias_dtype))
+        if gated:
+            assert_within(dg, want_dg, allowed(torch.float32, want_dg, dy.double().abs() * z.abs() * 1e-6 + 2.0**-23 * want_dg.abs()), (name, 'dgate'))
+        assert db is None or bool(torch.isfinite(db).all())
