@@ -11,7 +11,8 @@ namespace msamp {
 typedef int rows_v8i __attribute__((ext_vector_type(8)));
 typedef float rows_v4f __attribute__((ext_vector_type(4)));
 
-constexpr int kMostK = 1 << 26;    // offsets inside 32 rows of an operand are 32 bits
+constexpr int kMostK = 1 << 26;    // offsets inside the 64 rows of a workgroup are 32 bits
+constexpr long long kMostRows = 65535LL * 64;    // workgroups in a grid's second dimension, of 64 rows (so many are never taken by less)
 
 // Up to 16 * MB rows of D per workgroup, RB blocks of 16 columns of it.  The weight a is read once and everything else is small: what
 // bounds it is the weight's way from memory, and for the smallest weights the latency of a launch, of a load and of the sum.
@@ -317,29 +318,36 @@ extern "C" int msamp_fp8_gemm_fused(const msamp_gemm_fused_args* args, msamp_str
     ep.stream = static_cast<size_t>(a.n) * a.m * size >= (size_t(192) << 20);
     hipStream_t st = static_cast<hipStream_t>(stream);
     // The tile kernels fetch 16 bytes of a row at a time, at 32-bit offsets: a weight of 4 GiB and more is left to the other kernel, as
-    // are rows that begin anywhere; a longer x is taken in stretches of rows.
-    if (!takes_few_rows(a.n, a.m) && a.m * a.k < (1LL << 32) && a.k % 16 == 0 && aligned(a.a, 16) && aligned(a.b, 16)) {
-        const long long most = ((1LL << 32) - 1) / a.k / 16 * 16;
-        const size_t pitch = ckpt_pitch(static_cast<int>(a.m));
-        for (long long r = 0, rows; r < a.n; r += rows) {
-            rows = rows_in_front(std::min(most, a.n - r), static_cast<int>(a.m), static_cast<int>(a.k));
-            Epilogue e = ep;
-            auto byte = [](const void* p, long long n) { return p == nullptr ? nullptr : static_cast<const uint8_t*>(p) + n; };
-            auto code = [](uint8_t* p, size_t n) { return p == nullptr ? nullptr : p + n; };
-            e.gate = byte(ep.gate, r * ep.gate_ld * size), e.residual = byte(ep.residual, r * ep.residual_ld * size);
-            e.z_codes = code(ep.z_codes, r * pitch), e.z_exponents = code(ep.z_exponents, r * (pitch / kCkptBlock));
-            e.gate_codes = code(ep.gate_codes, r * pitch), e.gate_exponents = code(ep.gate_exponents, r * (pitch / kCkptBlock));
+    // are rows that begin anywhere.  A longer x is taken in stretches of rows, and so is one of more rows than the other kernel's
+    // grid has in its second dimension.
+    const bool tiles = !takes_few_rows(a.n, a.m) && a.m * a.k < (1LL << 32) && a.k % 16 == 0 && aligned(a.a, 16) && aligned(a.b, 16);
+    const long long most = tiles ? ((1LL << 32) - 1) / a.k / 16 * 16 : kMostRows;
+    const size_t pitch = ckpt_pitch(static_cast<int>(a.m));
+    for (long long r = 0, rows; r < a.n; r += rows) {
+        rows = std::min(most, a.n - r);
+        if (tiles) rows = rows_in_front(rows, static_cast<int>(a.m), static_cast<int>(a.k));
+        Epilogue e = ep;
+        auto byte = [](const void* p, long long n) { return p == nullptr ? nullptr : static_cast<const uint8_t*>(p) + n; };
+        auto code = [](uint8_t* p, size_t n) { return p == nullptr ? nullptr : p + n; };
+        e.gate = byte(ep.gate, r * ep.gate_ld * size), e.residual = byte(ep.residual, r * ep.residual_ld * size);
+        e.z_codes = code(ep.z_codes, r * pitch), e.z_exponents = code(ep.z_exponents, r * (pitch / kCkptBlock));
+        e.gate_codes = code(ep.gate_codes, r * pitch), e.gate_exponents = code(ep.gate_exponents, r * (pitch / kCkptBlock));
+        int done;
+        if (tiles) {
             const GemmCall c = {a.b + r * a.k, a.a, static_cast<uint8_t*>(a.d) + r * a.m * size, dt, static_cast<int>(rows),
                                 static_cast<int>(a.m), static_cast<int>(a.k), a.b_scale_inv, a.a_scale_inv, 0, a.bias,
                                 static_cast<int>(a.bias_dtype), false, false, nullptr, st};
-            const int done = dt == MSAMP_DT_F32   ? run_gemm_fused<float>(c, e)
-                             : dt == MSAMP_DT_F16 ? run_gemm_fused<f16_t>(c, e)
-                                                  : run_gemm_fused<bf16_t>(c, e);
-            if (done != MSAMP_OK) return done;
+            done = dt == MSAMP_DT_F32   ? run_gemm_fused<float>(c, e)
+                   : dt == MSAMP_DT_F16 ? run_gemm_fused<f16_t>(c, e)
+                                        : run_gemm_fused<bf16_t>(c, e);
+        } else {
+            msamp_gemm_fused_args part = a;
+            part.b = a.b + r * a.k, part.d = static_cast<uint8_t*>(a.d) + r * a.m * size, part.n = rows;
+            done = dt == MSAMP_DT_F32   ? run_rows<float>(part, e, st)
+                   : dt == MSAMP_DT_F16 ? run_rows<f16_t>(part, e, st)
+                                        : run_rows<bf16_t>(part, e, st);
         }
-        return MSAMP_OK;
+        if (done != MSAMP_OK) return done;
     }
-    if (dt == MSAMP_DT_F32) return run_rows<float>(a, ep, st);
-    if (dt == MSAMP_DT_F16) return run_rows<f16_t>(a, ep, st);
-    return run_rows<bf16_t>(a, ep, st);
+    return MSAMP_OK;
 }

@@ -581,3 +581,24 @@ def test_gradients_of_values_whose_square_leaves_float32(name, gated):
         if gated:
             assert_within(dg, want_dg, allowed(torch.float32, want_dg, dy.double().abs() * z.abs() * 1e-6 + 2.0**-23 * want_dg.abs()), (name, 'dgate'))
         assert db is None or bool(torch.isfinite(db).all())
+
+
+def test_more_rows_than_a_grid_has():
+    """Operands that begin anywhere, past 65535 workgroups of 64 rows: stretches, with their part of every operand."""
+    n, m, block = 65535 * 64 + 70, 3, 4096
+    x, xs = whole_codes(block, 1, 151)
+    w, ws = whole_codes(m, 1, 152)
+    codes = xs.value.repeat(n // block + 1, 1)[:n].contiguous()
+    gate = torch.randn(block, m, generator=gen(153)).bfloat16()
+    many = gate.cuda().repeat(n // block + 1, 1)[:n]
+    out, z8, g8 = torch.empty_like(many), BlockTensor._empty((n, m), many.device), BlockTensor._empty((n, m), many.device)
+    _backend.fp8_gemm_fused(ws.value, ws.meta.scale_inv, codes, xs.meta.scale_inv, out, None, _backend.activation_code('silu'), many, many, z8._pointers(),
+                            g8._pointers())
+    z = 0.0 + x.double() @ w.double().t() * 2.0**-10    # (a sum that begins at zero is no negative zero)
+    y = oact.value(z, 'silu') * gate.double() + gate.double()
+    assert_within(out[:block], y, allowed(torch.bfloat16, y, epilogue_error(z, gate, y, gate)), 'first block')
+    for packed, of in ((z8, z.float()), (g8, gate)):
+        want, exponents = oact.pack(of)
+        assert torch.equal(packed.value[:block].cpu(), want) and torch.equal(packed.exponent[:block].cpu(), exponents)
+        assert same_blocks(packed.value, block) and same_blocks(packed.exponent, block)
+    assert same_blocks(out, block)
