@@ -144,6 +144,10 @@ class _FP8GemmFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, output_grad):
+        return _FP8GemmFunction._gradients(ctx, output_grad, ctx.need_bias_grad)
+
+    @staticmethod
+    def _gradients(ctx, output_grad, need_bias_grad):
         output_grad = output_grad.contiguous()
         metas = ctx.metas
         tokens, d_out = output_grad.shape
@@ -166,7 +170,7 @@ class _FP8GemmFunction(torch.autograd.Function):
             in_place = _backend.linear_takes_short_k(tokens, d_in, d_out) and _backward_in_one_call(ctx, output_grad, d_in, need_dgrad)
         words = ctx.weight_words
         input_grad = bias_grad = None
-        column_sums = in_place and ctx.need_bias_grad and TypeCast.takes_column_sums(output_grad, metas['ograd'], ctx.bias_dtype)
+        column_sums = in_place and need_bias_grad and TypeCast.takes_column_sums(output_grad, metas['ograd'], ctx.bias_dtype)
         if in_place and _backward_in_one_call(ctx, output_grad, d_in, need_dgrad):
             # (a weight gradient that is cast inside its product keeps a call of its own)
             with_wgrad = need_wgrad and _wgrad_in_one_call(ctx, tokens, d_in, d_out)
@@ -194,7 +198,7 @@ class _FP8GemmFunction(torch.autograd.Function):
             if need_dgrad:
                 input_grad = grad
 
-        if ctx.need_bias_grad and bias_grad is None:
+        if need_bias_grad and bias_grad is None:
             bias_grad = output_grad.sum(0).to(ctx.bias_dtype)
         return input_grad, None, None, None, bias_grad, None
 
@@ -286,7 +290,7 @@ class _FP8FusedLinearFunction(torch.autograd.Function):
             input_grad = _FP8GemmFunction._products(ctx, ograd_fp8, None, True, ctx.input_codes, ctx.weight_codes, need_dgrad, need_wgrad)
         else:    # a shape whose products want transposed copies, or a meta without a window
             preact_grad, gate_grad, bias_grad = Activation.backward(output_grad, ctx.z, ctx.activation, gate=ctx.gate, bias_dtype=bias_dtype)
-            input_grad = _FP8GemmFunction.backward(ctx, preact_grad)[0]
+            input_grad = _FP8GemmFunction._gradients(ctx, preact_grad, False)[0]
         return input_grad, None, None, None, bias_grad, None, gate_grad if need_gate_grad else None, \
             output_grad if need_residual_grad else None, None
 

@@ -9,7 +9,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 
 import msamp
 from msamp.common.dtype import Dtypes
-from msamp.common.tensor import ScalingMeta
+from msamp.common.tensor import ScalingMeta, TypeCast
 from msamp.nn import FeedForward, FP8Linear, LinearReplacer, model_state, saved_in_8_bits
 from msamp.nn.functional import linear_fused
 from msamp.optim import LBAdamW
@@ -348,3 +348,38 @@ def test_backward_frees_what_the_forward_pass_kept(d_in, d_out):
     codes = tokens * d_out * 2 * 33 // 32
     held, left = kept[-1]
     assert held > codes and left < y_bytes + grads + (1 << 20)
+
+
+@pytest.mark.parametrize('tokens,d_in,d_out', [(64, 128, 256), (33, 200, 99), (300, 100, 60), (512, 64, 1040)])
+@pytest.mark.parametrize('form', ['no window', 'no window, frozen weight', 'fp8 ddp', 'fp8 ddp, no window'])
+def test_backward_of_the_layer_by_its_other_ways(tokens, d_in, d_out, form, monkeypatch):
+    """Metas without a window (casts apart from the gradients), operands that the products want transposed, gradients that a data-parallel
+    reducer casts: against 64 bits of the unquantized layer, one backward pass behind another."""
+    layer = fp8_layer(d_in, d_out, torch.bfloat16, seed=tokens)
+    if 'no window' in form:
+        for name in ('input', 'ograd'):
+            layer.scaling_metas[name].window_size = 1
+    if 'frozen' in form:
+        layer.weight.requires_grad = False
+    model_state.use_fp8_ddp = 'ddp' in form
+    taken = []
+    take = TypeCast.takes_column_sums
+    monkeypatch.setattr(TypeCast, 'takes_column_sums', staticmethod(lambda *args: taken.append(1) or take(*args)))
+    x = torch.randn(tokens, d_in, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    gate = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16)
+    for _ in range(2):
+        layer(x, activation='silu', gate=gate).backward(dy)
+    assert not taken    # (the bias' gradient is there before)
+
+    x64, g64, b64 = (t.detach().double().cpu().requires_grad_(True) for t in (x, gate, layer.bias))
+    w64 = (layer.weight.value.double().cpu() * float(layer.weight.meta.scale_inv)).requires_grad_(True)
+    (torch.nn.functional.silu(x64 @ w64.t() + b64) * g64).backward(2 * dy.double().cpu())
+    product = 2 * (2 * E4M3_RMS**2)**0.5
+    grads = 2 * (E5M2_RMS**2 + 3 * E4M3_RMS**2)**0.5 + product
+    assert rel_fro(x.grad, x64.grad) < grads and rel_fro(gate.grad, g64.grad) < grads and rel_fro(layer.bias.grad, b64.grad) < grads
+    if 'frozen' in form:
+        assert layer.weight.grad is None
+    else:
+        assert isinstance(layer.weight.grad, torch.Tensor) == ('ddp' in form)
+        assert rel_fro(layer.weight.grad.float(), w64.grad) < grads + 2 * E4M3_RMS    # (two casts of it)
