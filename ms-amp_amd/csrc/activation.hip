@@ -25,8 +25,7 @@ static Divisor divisor_of(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor& v) { return __umulhi(n, v.m) >> v.shift; }
 
-// Where eight number idx of the checkpoint lies: rows of `eights` eights, `cols` values of them real.  `flat`: rows that follow one
-// another without a gap, in memory and in the checkpoint, are one.
+// Where eight number idx of the checkpoint lies: rows of `eights` eights, `cols` values of them real.
 struct Place {
     size_t row;
     int col, valid;
@@ -34,7 +33,6 @@ struct Place {
 struct Rows {
     Divisor eights;
     int cols;
-    int flat;
 };
 __device__ __forceinline__ Place place_of(uint32_t idx, const Rows& r) {
     const uint32_t row = quotient(idx, r.eights);
@@ -142,7 +140,6 @@ struct Slabs {
     int lanes_log2;
     int rows;
 };
-
 
 struct __attribute__((packed, aligned(1))) Anywhere8 {
     uint2 v;
@@ -411,9 +408,6 @@ __global__ __launch_bounds__(kActThreads) void gradient_top_kernel(GradientArgs 
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// Rows that follow one another without a gap, in whole blocks, are one row.
-static bool one_row(long long cols, long long ld) { return cols % kCkptBlock == 0 && ld == cols; }
-
 // calls f(first row, rows of it, total eights) for stretches of rows whose eights are counted in 31 bits
 template <typename F>
 static int in_stretches(long long rows, int cols, F&& f) {
@@ -430,7 +424,7 @@ template <typename T>
 static int launch_pack(const T* x, long long rows, int cols, long long ld, uint8_t* codes, uint8_t* exponents, hipStream_t st) {
     const bool vec = cols % 8 == 0 && ld * sizeof(T) % 16 == 0 && aligned(x, 16);
     const size_t pitch = ckpt_pitch(cols);
-    const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols, 0};
+    const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols};
     return in_stretches(rows, cols, [&](long long r, long long, uint32_t total) {
         const dim3 grid((total + kActThreads - 1) / kActThreads);
         const auto kern = vec ? ckpt_pack_kernel<T, true> : ckpt_pack_kernel<T, false>;
@@ -444,7 +438,7 @@ template <typename T>
 static int launch_unpack(const uint8_t* codes, const uint8_t* exponents, long long rows, int cols, T* out, hipStream_t st) {
     const bool vec = cols % 8 == 0 && aligned(out, 16);
     const size_t pitch = ckpt_pitch(cols);
-    const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols, 0};
+    const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols};
     return in_stretches(rows, cols, [&](long long r, long long, uint32_t total) {
         const dim3 grid((total + kActThreads - 1) / kActThreads);
         const auto kern = vec ? ckpt_unpack_kernel<T, true> : ckpt_unpack_kernel<T, false>;
@@ -477,7 +471,7 @@ static int launch_gradient(const msamp_activation_backward_args& a, const Gradie
     const int fmt = static_cast<int>(a.dz_type);
     if (!is_fp8(fmt) && a.bias_sum == nullptr) {
         const size_t pitch = ckpt_pitch(cols);
-        const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols, 0};
+        const Rows shape = {divisor_of(static_cast<uint32_t>(pitch / 8)), cols};
         return in_stretches(rows, cols, [&](long long r, long long, uint32_t total) {
             GradientArgs p = g;
             p.dy = static_cast<const T*>(g.dy) + r * g.dy_ld;

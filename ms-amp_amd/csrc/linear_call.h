@@ -16,7 +16,6 @@ int cast_output_gradient(const msamp_linear_backward_args& a, void* product, flo
 int few_cast_fragments(const void* x, int in_dtype, int tokens, int K, float* scale, float* amax, float* scale_inv, uint8_t* out,
                        int flags, const int32_t* counter, int window, void* workspace, hipStream_t st);
 
-
 // what msamp_fp8_gemm_fused refuses
 int check_gemm_fused(const msamp_gemm_fused_args& a);
 
