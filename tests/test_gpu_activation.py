@@ -602,3 +602,33 @@ def test_more_rows_than_a_grid_has():
         assert torch.equal(packed.value[:block].cpu(), want) and torch.equal(packed.exponent[:block].cpu(), exponents)
         assert same_blocks(packed.value, block) and same_blocks(packed.exponent, block)
     assert same_blocks(out, block)
+
+
+# (few rows in 16-byte accesses and not; paired, small and large tiles, whole and ragged slices of K; tiles of two sizes; rows that begin anywhere in tiles)
+@pytest.mark.parametrize('n,m,k', [(1, 1000, 1040), (48, 300, 200), (130, 512, 512), (2048, 1024, 1024), (1024, 1032, 2064), (2304, 8192, 400), (4289, 4096, 2048),
+                                   (2500, 4101, 384)])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_fused_product_of_sums_that_round(n, m, k, dtype):
+    """Codes of every size.  The FP8 matrix instruction itself sums to some 16 bits: 1.5e-5 of a product's norm (measured on random
+    operands, whatever K).  Of normal values an error is that of the product's spread, |x| |w| / sqrt(K) of its row and its column, and
+    32 times it is allowed to a single output (2^-11), 6 times it to the norm."""
+    xs, ws = (ScalingTensor((torch.randn(rows, k, generator=gen(s)) * 60.0).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).cuda(),
+                            ScalingMeta(Dtypes.kfloat8_e4m3, scale_inv=torch.tensor(inv, device='cuda')))
+              for rows, s, inv in ((n, 161, 0.013), (m, 162, 0.0007)))
+    x, w = (t.value.view(torch.float8_e4m3fn).double() * t.meta.scale_inv.double() for t in (xs, ws))
+    product = (x @ w.t()).cpu()
+    off = 2.0**-11 * (x.norm(dim=1)[:, None] * w.norm(dim=1)[None, :]).cpu() / math.sqrt(k)
+    plain = Gemm.fp8_gemm_fused(ws, xs, Dtypes.kfloat32).double().cpu()
+    assert float((plain - product).norm()) <= 6 * 1.5e-5 * float(product.norm())
+    bias, gate, residual = (torch.randn(shape, generator=gen(s)).to(dtype) for shape, s in (((m, ), 163), ((n, m), 164), ((n, m), 165)))
+    z = product + bias.double()
+    out, z8, g8 = Gemm.fp8_gemm_fused(ws, xs, Dtypes.dtype_to_qtype[dtype], bias=bias.cuda(), activation='gelu', gate=gate.cuda(), residual=residual.cuda(),
+                                      checkpoint=True)
+    y = oact.value(z, 'gelu') * gate.double() + residual.double()
+    off = off + 2.0**-23 * z.abs()
+    # (GELU's slope is at most 1.13)
+    assert_within(out, y, allowed(dtype, y, epilogue_error(z, gate, y, residual) + 1.13 * off * gate.double().abs()), (n, m, k, dtype))
+    assert_packed(g8, gate)
+    block = oact.blocks(z).abs().amax(2).repeat_interleave(32, 1)[:, :m]
+    bound = torch.maximum(z.abs() / 16, block / 448 * 2.0**-9) + 2 * off
+    assert_within(z8.float(), z, bound, 'checkpoint')
