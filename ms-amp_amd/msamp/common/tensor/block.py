@@ -99,12 +99,16 @@ class BlockTensor:
         return self.shape.numel()
 
     @property
+    def _codes(self):
+        return self._value if self._buffer is None else self._buffer
+
+    @property
     def device(self):
-        return (self._value if self._buffer is None else self._buffer).device
+        return self._codes.device
 
     @property
     def is_cuda(self):
-        return (self._value if self._buffer is None else self._buffer).is_cuda
+        return self._codes.is_cuda
 
     @property
     def nbytes(self):

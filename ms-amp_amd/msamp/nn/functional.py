@@ -225,8 +225,8 @@ class _FP8FusedLinearFunction(torch.autograd.Function):
         keeps = differentiable and (activation is not None or gate is not None)
         if _casts_in_one_call(src, meta, weight, output_dtype, bias):
             (n, m), device = (src.shape[0], weight.shape[0]), src.device
-            gate = None if gate is None else Gemm._beside_output(gate, 'gate', n, m, output_dtype, device)
-            residual = None if residual is None else Gemm._beside_output(residual, 'residual', n, m, output_dtype, device)
+            gate = None if gate is None else Gemm._beside_output(gate, 'gate', n, m, output_dtype, device.index)
+            residual = None if residual is None else Gemm._beside_output(residual, 'residual', n, m, output_dtype, device.index)
             if keeps:
                 z = BlockTensor._empty((n, m), device)
                 g = None if gate is None else BlockTensor._empty((n, m), device)

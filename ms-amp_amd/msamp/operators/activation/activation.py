@@ -18,10 +18,9 @@ class Activation:
     def _checked(output_grad, z, gate, bias_dtype):
         if not isinstance(z, BlockTensor) or not (gate is None or isinstance(gate, BlockTensor)):
             raise TypeError('z and the gate should be BlockTensors.')
-        if not (output_grad.is_cuda and z.is_cuda and (gate is None or gate.is_cuda)):
-            raise ValueError('The output gradient or a checkpoint is not in cuda memory.')
-        if z.device != output_grad.device or gate is not None and gate.device != output_grad.device:
-            raise ValueError('The output gradient and the checkpoints are on different devices.')
+        gpu = output_grad.get_device()    # (-1 in host memory)
+        if gpu < 0 or z._codes.get_device() != gpu or gate is not None and gate._codes.get_device() != gpu:
+            raise ValueError('The output gradient and the checkpoints are not all on one GPU.')
         if output_grad.dtype not in _FLOATS or bias_dtype not in _FLOATS + (None, ):
             raise TypeError(f'unsupported types: output gradient {output_grad.dtype}, bias gradient {bias_dtype}.')
         if output_grad.shape != z.shape or gate is not None and gate.shape != z.shape:

@@ -123,16 +123,14 @@ class Gemm:
         return out
 
     @staticmethod
-    def _beside_output(tensor, what, n, m, dtype, device):
+    def _beside_output(tensor, what, n, m, dtype, gpu):
         """A gate or residual as the kernel takes it: [N, M] in the output's type, its rows contiguous, any distance apart."""
         if tensor.shape != (n, m):
             raise ValueError(f'the {what} has shape {tuple(tensor.shape)}, the output ({n}, {m}).')
         if tensor.dtype != dtype:
             raise TypeError(f'the {what} is {tensor.dtype}, the output {dtype}.')
-        if not tensor.is_cuda:
-            raise ValueError(f'The {what} is not in cuda memory.')
-        if tensor.device != device:
-            raise ValueError(f'The {what} is on {tensor.device}, the operands on {device}.')
+        if tensor.get_device() != gpu:
+            raise ValueError(f'The {what} is on {tensor.device}, the operands on cuda:{gpu}.')
         return tensor if tensor.stride(1) == 1 and (n == 1 or tensor.stride(0) >= m) else tensor.contiguous()
 
     @classmethod
@@ -156,20 +154,21 @@ class Gemm:
         (m, k), (n, b_k), device = a.shape, b.shape, a.device
         if k != b_k or k == 0:
             raise ValueError(f'shape mismatch: mat_a {tuple(a.shape)}, mat_b {tuple(b.shape)}.')
-        if not (a.is_cuda and a.is_contiguous() and b.is_cuda and b.is_contiguous()):
+        gpu = a.get_device()    # (-1 in host memory; a number is compared in half the time of a device)
+        if gpu < 0 or not (a.is_contiguous() and b.is_contiguous()):
             raise ValueError('The operands are not in cuda memory or contiguous.')
-        if b.device != device or a_meta.scale_inv.device != device or b_meta.scale_inv.device != device:
+        if b.get_device() != gpu or a_meta.scale_inv.get_device() != gpu or b_meta.scale_inv.get_device() != gpu:
             raise ValueError('The operands and their reciprocal scales are not all on one device.')
         code = _backend.activation_code(activation)
         dtype = cls._FLOATS.get(int(out_qtype))
         if dtype is None:
             raise TypeError(f'the output should be float32, float16 or bfloat16, not {out_qtype}.')
-        if bias is not None and not (bias.device == device and bias.is_contiguous() and bias.numel() == m):
-            raise ValueError(f'The bias is not on {device}, not contiguous or not of {m} values.')
+        if bias is not None and not (bias.get_device() == gpu and bias.is_contiguous() and bias.numel() == m):
+            raise ValueError(f'The bias is not on cuda:{gpu}, not contiguous or not of {m} values.')
         if gate is not None:
-            gate = cls._beside_output(gate, 'gate', n, m, dtype, device)
+            gate = cls._beside_output(gate, 'gate', n, m, dtype, gpu)
         if residual is not None:
-            residual = cls._beside_output(residual, 'residual', n, m, dtype, device)
+            residual = cls._beside_output(residual, 'residual', n, m, dtype, gpu)
         out = torch.empty((n, m), dtype=dtype, device=device)
         z = g = None
         if checkpoint:
