@@ -1,10 +1,11 @@
 """Trains a gated feed-forward block twice, as msamp.nn.FeedForward and as FP8 linear layers with torch's operators between them:
-loss, time of a step and memory held for the backward pass.
+loss, time of a step, memory held between the forward and the backward pass and the most that a step takes.
 
     python examples/feed_forward.py [--tokens 16384] [--width 4096] [--hidden 11008] [--steps 20]
 """
 
 import argparse
+import gc
 import os
 import sys
 import time
@@ -54,10 +55,16 @@ def train(fused, args):
     target = torch.roll(x, 1, dims=1)
     held = 0
     for step in range(args.steps):
+        if step == args.steps // 2 - 5:
+            gc.collect()    # (a collection of all generations takes some 80 ms: not in the steps that are timed, nor right before them)
         if step == args.steps // 2:
             torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
             began = time.perf_counter()
         optimizer.zero_grad()
+        if step == 1:    # the model, the optimizer's state and the data, without the last step's loss and what hangs on it
+            y = loss = None
+            stands = torch.cuda.memory_allocated()
         before = torch.cuda.memory_allocated()
         y = model(x)
         held = torch.cuda.memory_allocated() - before
@@ -65,8 +72,10 @@ def train(fused, args):
         loss.backward()
         optimizer.step()
     torch.cuda.synchronize()
+    most = torch.cuda.max_memory_allocated() - stands
     ms = (time.perf_counter() - began) / (args.steps - args.steps // 2) * 1e3
-    print(f'{"fused" if fused else "plain"}: loss {float(loss.detach()):.4f}, {ms:.2f} ms a step, {held / 2**20:.0f} MiB held after the forward pass', flush=True)
+    print(f'{"fused" if fused else "plain"}: loss {float(loss.detach()):.4f}, {ms:.2f} ms a step, {held / 2**20:.0f} MiB held after the forward pass, '
+          f'{most / 2**20:.0f} MiB at most beside model and optimizer', flush=True)
 
 
 if __name__ == '__main__':
