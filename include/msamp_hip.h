@@ -632,7 +632,7 @@ int msamp_checkpoint_unpack(const uint8_t* codes, const uint8_t* exponents, long
 
 /* d[n][m] = act(z) * gate + residual with z = (b[n][k] . a[m][k]^T) * a_scale_inv * b_scale_inv + bias, rounded once to d_dtype;
  * a and b are E4M3 codes, z and all behind it float32.  gate and residual: rows of d's type, their strides in elements; the
- * residual may be d.  z_codes / gate_codes: checkpoints of z (rounded from float32) and of the gate, written beside d.
+ * residual may be d (its rows m apart then), the gate may not.  z_codes / gate_codes: checkpoints of z (rounded from float32) and of the gate, written beside d.
  * Every n, m >= 1 and k from 1 to 2^26, a and b aligned in any way.  Up to MSAMP_FUSED_ROWS rows, and more of them where d is small,
  * any k is as good as another; else rows of k a multiple of 16, which msamp_fp8_gemm_fused_pitch asks for, are several times faster.
  * msamp_pad_codes makes them: the rows of a and of b with zeros behind the last code, 16-byte aligned. */

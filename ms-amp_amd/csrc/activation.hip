@@ -493,7 +493,8 @@ static int launch_gradient(const msamp_activation_backward_args& a, const Gradie
     if (is_fp8(fmt)) {
         const Gate gate = {a.counter, static_cast<int>(a.window)};
         const Finish fin = {a.amax, a.scale, a.scale_inv, fp8_max(fmt), 0, 0};
-        // (as a rule the gate is closed and its workgroups return at once: few of them)
+        // (As a rule the gate is closed and its workgroups return at once: few of them.  While the window fills they read everything once
+        // more, slowly: bfloat16, GELU, bias, to E5M2 12605 x 4304 120 us instead of 46, 16384 x 11008 436 instead of 144.)
         const SlabGrid few = slab_grid(rows, cols, std::min(cu_count(), kMaxPartials));
         hipLaunchKernelGGL((gradient_top_kernel<T, VEC, GATED>), dim3(few.strips, few.slabs), dim3(kActThreads), 0, st, g, cols, few.s, gate, fin,
                            static_cast<uint32_t*>(a.workspace));

@@ -176,7 +176,9 @@ static int launch_rows(const msamp_gemm_fused_args& a, const Epilogue& ep, hipSt
 // so fewer of them cost less, while all compute units have one.  us with 1, 2, 3 and 4 blocks, bfloat16 with a gate, on 256 compute units:
 //   48 x 4096 -> 12288 (3 blocks a unit)  13.7, 13.0, 11.6, 12.1    64 x 4096 -> 11008 (2.7)  15.2, 15.4, 12.3, 12.9
 //   33 x 4096 -> 16384 (4)                16.3, 14.2, 17.7, 14.1    48 x 11008 -> 4096 (1)    12.0, 13.9, 16.3, 18.8
-//   1 x 4096 -> 11008                      9.8, 10.1,  -,    9.3    1 x 11008 -> 4096          9.4, 10.2,  -,   11.9
+// the same with the weights of twelve layers in turn, so that they come from memory:
+//   1 x 4096 -> 11008 (2.7)               11.1, 11.8, 10.5, 10.7    1 x 11008 -> 4096 (1)     11.9, 12.8, 14.8, 18.1
+//   1 x 4096 -> 12288 (3)                 11.9, 12.1, 11.3, 11.4    16 x 4096 -> 11008 (2.7)  11.8, 12.8, 10.7, 11.1
 static int column_blocks(long long cols) {
     return static_cast<int>(std::min<long long>(4, ((cols + 15) / 16 + cu_count() - 1) / cu_count()));
 }

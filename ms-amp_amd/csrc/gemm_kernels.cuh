@@ -858,7 +858,10 @@ __device__ __forceinline__ void gemm_dma256(const uint8_t* __restrict__ X, const
                     work(p + kFusedGroup, next, other);
                 }
             });
-        } else {    // rows that begin anywhere or end inside an eight: one at a time
+        } else {
+            // Rows that begin anywhere or end inside an eight: one at a time, and every load behind every store before it, which shows where
+            // the epilogue reads much.  bfloat16, us, here | at the next multiple of 8: 8192 x 4096 -> 50257 with a bias 1382 | 1212,
+            // -> 4099 with a residual 156 | 120, -> 11003 with SiLU and a gate 485 | 300.
             static_for<2>([&](auto wc_) {
                 constexpr int w = decltype(wc_)::value;
                 dump(wc_);

@@ -464,7 +464,7 @@ __device__ __forceinline__ void gemm_dma128(const uint8_t* __restrict__ X, const
                     }
                 }
             });
-        } else {    // rows that begin anywhere or end inside an eight
+        } else {    // rows that begin anywhere or end inside an eight: one at a time, as in the large tile
             dump();
 #pragma unroll 1
             for (int p = 0; p < kPasses; ++p) {

@@ -305,7 +305,9 @@ def linear_fused(input, weight, bias=None, activation=None, gate=None, residual=
 
     activation: None, 'relu', 'gelu', 'gelu_tanh' or 'silu'.  gate, residual: tensors of the output's shape (converted to its
     type if they are not); a 2-D view whose rows lie apart, such as a half of a wider tensor, is read in place.  Where a gradient is
-    recorded and there is an activation or a gate, the pre-activation and the gate are kept in 8 bits (BlockTensor) and nothing in 16."""
+    recorded and there is an activation or a gate, the pre-activation and the gate are kept in 8 bits (BlockTensor) and nothing in 16.
+    The weight is cast on every call; of up to 64 tokens without a gradient the plain layer does not need its codes, and with
+    torch's operators behind it takes less (4096 -> 12288, SiLU and a gate, us, here | so: 1 token 46 | 38, 64 52 | 47; 256 57 | 65)."""
     if not isinstance(input, torch.Tensor):
         raise TypeError(f'input should be a torch.Tensor. current type: {type(input)}')
     if not isinstance(weight, ScalingTensor) or not hasattr(weight, '_scaling_metas'):

@@ -142,6 +142,8 @@ class Gemm:
         and rounded once, to out_qtype (kfloat32, kfloat16 or kbfloat16).
         bias: [M], any of these types.  activation: None, 'relu', 'gelu', 'gelu_tanh' or 'silu'.  gate, residual: [N, M] in the
         output's type; their rows may lie apart (a half of a wider tensor).
+        Of what a float32 output shows: the FP8 matrix instruction sums its products to some 16 bits (1.5e-5 of a product's norm, whatever
+        K), and GELU is held to an absolute 4e-7, so its far negative side has no relative accuracy.
         With `checkpoint` the call returns (out, z8, gate8): BlockTensors with the 8-bit checkpoints of z and of the gate (None
         without one), written on the way, from which Activation.backward takes the gradients.  Not recorded by autograd."""
         if not (isinstance(mat_a, ScalingTensor) and isinstance(mat_b, ScalingTensor)):
