@@ -43,6 +43,11 @@ def _on_gpu(tensor):
     return tensor.is_cuda
 
 
+def _dense(tensor):
+    """A tensor whose values lie in memory of its own: not a sparse or nested one, and no subclass, whose memory need not be what it shows."""
+    return type(tensor) in (torch.Tensor, torch.nn.Parameter) and tensor.layout == torch.strided and not tensor.is_nested
+
+
 def _of_leaf(tensor):
     """A parameter, another leaf that wants a gradient, or either in another type or shape."""
     if isinstance(tensor, torch.nn.Parameter) or isinstance(tensor._base, torch.nn.Parameter):
@@ -81,8 +86,7 @@ class _Operators(TorchFunctionMode):
                 held, key = (args, at) if at < len(args) else (kwargs, name)
                 x = args[at] if held is args else kwargs.get(name)
                 # (of several factors one without a gradient is a mask, a table or a frozen weight)
-                if not isinstance(x, torch.Tensor) or x.layout != torch.strided or not _on_gpu(x) or several and not x.requires_grad or \
-                        _of_leaf(x):
+                if not isinstance(x, torch.Tensor) or not _dense(x) or not _on_gpu(x) or several and not x.requires_grad or _of_leaf(x):
                     continue
                 # Autocast would make a copy of its own, which could not be told from one of a weight.
                 if autocast is not None and x.dtype in _FLOATS and torch.is_autocast_enabled(x.device.type):
@@ -107,16 +111,17 @@ class saved_in_8_bits(torch.autograd.graph.saved_tensors_hooks):
     RMS norms, GELU, SiLU, Mish, GLU and leaky ReLU, and for ReLU's result, where a program calls them on activations.  Left as they are:
     whatever other operators save (attention's inputs and statistics, logarithms, probabilities, a custom autograd function's own), the
     statistics of norms, parameters, views of them and copies in another type (autocast's among them), other leaves that want a gradient,
-    factors that want none, and tensors that are not float32, float16 or bfloat16 on the GPU, of fewer than min_numel values, or
-    whose last dimension is shorter than a block of 32.  A tensor that several operators save is held once for each of them.  What
-    FP8Linear layers keep is in 8 bits already."""
+    factors that want none, sparse and nested tensors and subclasses, and tensors that are not float32, float16 or bfloat16 on the GPU, of
+    fewer than min_numel values, or whose last dimension is shorter than a block of 32.  A tensor that several operators save is held
+    once for each of them.  What FP8Linear layers keep is in 8 bits already.  (A weight that is computed from others is an activation
+    like any other, unless it is a linear layer's or a convolution's.)"""
 
     def __init__(self, min_numel=1 << 16):
         self._operators = operators = _Operators()
 
         def pack(tensor):
             packs = operators.packs
-            if packs is not _ALL and (not packs or tensor.untyped_storage().data_ptr() not in packs) or not _on_gpu(tensor) or \
+            if not packs or not _dense(tensor) or packs is not _ALL and tensor.untyped_storage().data_ptr() not in packs or not _on_gpu(tensor) or \
                     tensor.dtype not in _FLOATS or tensor.numel() < min_numel or tensor.dim() == 0 or not 32 <= tensor.shape[-1] <= _backend.CKPT_COLS:
                 # (detached: an operator's result would hold the operator, and so itself.  Autograd takes no note of versions behind hooks.)
                 return tensor.detach(), tensor._version

@@ -203,3 +203,24 @@ def test_changes_in_place_are_noticed():
     want, = torch.autograd.grad(y.sum(), x, retain_graph=True)
     h.detach().zero_()
     assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
+
+
+class Other(torch.Tensor):
+    """A subclass, whose memory need not be what it shows."""
+
+
+def test_other_kinds_of_tensors_are_left_alone():
+    x, w = rand(96, 96, seed=31, grad=False).relu(), rand(96, 96, seed=32)
+    sparse = x.to_sparse().requires_grad_(True)
+    for f in (lambda: torch.mm(sparse * 1.0, w * 1.0).sum(), lambda: (torch.sparse.mm(sparse, w * 1.0) * 2.0).sum(),
+              lambda: torch.relu(torch.nested.nested_tensor([w[:3], w[3:7]], requires_grad=True)).to_padded_tensor(0.0).sum(),
+              lambda: F.gelu((w * 1.0).as_subclass(Other)).sum()):
+        w.grad = None
+        f().backward()
+        want, w.grad = w.grad, None
+        Rounded.taken = []
+        with saved_in_8_bits(min_numel=1):
+            loss = f()
+        loss.backward()
+        assert all(shape == (96, 96) for shape, _ in Rounded.taken)
+        assert (w.grad is None) == (want is None) and (want is None or bool(Rounded.taken) or torch.equal(w.grad, want))
