@@ -53,8 +53,8 @@ class BlockTensor:
             rows = tensor.detach()
             rows = rows.reshape(-1, cols) if tensor.numel() else rows.new_empty(shape[:-1].numel(), cols)
         n, cols = rows.shape
-        if cols > 1 and rows.stride(1) != 1 or n > 1 and rows.stride(0) < cols:
-            rows = rows.detach().contiguous()
+        if cols > 1 and rows.stride(1) != 1 or n > 1 and rows.stride(0) < cols or rows.is_neg():
+            rows = rows.detach().resolve_neg().contiguous()
         return cls._empty(shape, rows.device, n, _backend.checkpoint_pack(rows))
 
     def _pointers(self):

@@ -32,8 +32,8 @@ class Activation:
         cols = dy.shape[-1]
         if dy.numel() and dy.dim() != 2:
             dy = dy.detach().reshape(-1, cols)
-        if dy.numel() and (cols > 1 and dy.stride(1) != 1 or dy.shape[0] > 1 and dy.stride(0) < cols):
-            dy = dy.detach().contiguous()
+        if dy.numel() and (cols > 1 and dy.stride(1) != 1 or dy.shape[0] > 1 and dy.stride(0) < cols or dy.is_neg()):
+            dy = dy.detach().resolve_neg().contiguous()
         return dy
 
     @classmethod

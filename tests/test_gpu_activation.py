@@ -632,3 +632,18 @@ def test_fused_product_of_sums_that_round(n, m, k, dtype):
     block = oact.blocks(z).abs().amax(2).repeat_interleave(32, 1)[:, :m]
     bound = torch.maximum(z.abs() / 16, block / 448 * 2.0**-9) + 2 * off
     assert_within(z8.float(), z, bound, 'checkpoint')
+
+
+def test_lazily_negated_values_are_read_as_what_they_are():
+    """The imaginary part of a conjugate is a view of the original's with a mark that its sign is turned; of a single column nothing
+    else tells it from rows that lie apart."""
+    for cols in (1, 96):
+        c = torch.randn(64, cols, device='cuda', dtype=torch.complex64)
+        view, side = c.conj().imag, -torch.view_as_real(c)[..., 1].contiguous()
+        assert view.is_neg() and torch.equal(view, side)
+        assert_packed(BlockTensor.pack(view), side.cpu())
+        z8, z = held(64, cols, 171)
+        assert torch.equal(Activation.backward(view, z8, 'silu')[0], Activation.backward(side, z8, 'silu')[0])
+        x, xs = whole_codes(64, 256, 172)
+        w, ws = whole_codes(cols, 256, 173)
+        assert torch.equal(Gemm.fp8_gemm_fused(ws, xs, Dtypes.kfloat32, gate=view, residual=view), Gemm.fp8_gemm_fused(ws, xs, Dtypes.kfloat32, gate=side, residual=side))
