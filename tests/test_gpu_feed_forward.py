@@ -5,6 +5,7 @@ import copy
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 import msamp
@@ -383,3 +384,28 @@ def test_backward_of_the_layer_by_its_other_ways(tokens, d_in, d_out, form, monk
     else:
         assert isinstance(layer.weight.grad, torch.Tensor) == ('ddp' in form)
         assert rel_fro(layer.weight.grad.float(), w64.grad) < grads + 2 * E4M3_RMS    # (two casts of it)
+
+
+@pytest.mark.parametrize('d_in,d_out', [(256, 512), (200, 99)])
+def test_layer_with_an_epilogue_under_hooks_of_autograd(d_in, d_out):
+    """Activation checkpointing, which runs the forward pass again, and saved tensors that go to the host and back: the same gradients."""
+    tokens = 160
+    grads = []
+    for how in ('plain', 'again', 'host', '8 bits'):
+        model_state.clear()
+        layer = fp8_layer(d_in, d_out, torch.bfloat16, seed=2)
+        torch.manual_seed(3)
+        x = torch.randn(tokens, d_in, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+        gate = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+        dy = torch.randn(tokens, d_out, device='cuda', dtype=torch.bfloat16)
+        call = lambda x, gate: layer(x, activation='gelu', gate=gate)    # noqa: E731
+        if how == 'again':
+            y = torch.utils.checkpoint.checkpoint(call, x, gate, use_reentrant=False)
+        else:
+            with {'plain': contextlib.nullcontext, 'host': torch.autograd.graph.save_on_cpu, '8 bits': lambda: saved_in_8_bits(min_numel=1)}[how]():
+                y = call(x, gate)
+        y.backward(dy)
+        grads.append([y.detach(), x.grad, gate.grad, layer.bias.grad, layer.weight.grad.value])
+    for other in grads[1:]:
+        for a, b in zip(other, grads[0]):
+            assert torch.equal(a, b)
