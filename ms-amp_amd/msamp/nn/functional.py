@@ -251,8 +251,9 @@ class _FP8FusedLinearFunction(torch.autograd.Function):
     def backward(ctx, output_grad):
         ctx.input_codes, ctx.weight_codes, words, z, gate = ctx.saved_tensors
         ctx.weight_words = ctx.weight_meta if words is None else words
-        shape, device = output_grad.shape, output_grad.device
-        ctx.z, ctx.gate = (None if buffer is None else BlockTensor._empty(shape, device, buffer=buffer) for buffer in (z, gate))
+        shape = output_grad.shape
+        ctx.z = None if z is None else BlockTensor._empty(shape, None, shape[0], z)
+        ctx.gate = None if gate is None else BlockTensor._empty(shape, None, shape[0], gate)
         try:
             return _FP8FusedLinearFunction._gradients(ctx, output_grad)
         finally:
